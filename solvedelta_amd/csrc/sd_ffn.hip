@@ -107,6 +107,9 @@ struct EpiDact : EpiNothing {
     const bool ok = m < M;
     store_block(dg, m, ok, nb, N, vg);
     store_block(du, m, ok, nb, du.ld - N, vu);
+    // the row's end may lie up to 3 columns behind the last block (N = 29 to 31 of 32)
+    if (ok && nb + 32 >= N)
+      for (int64_t n = nb + 32 + (lane_id() >> 5); n < du.ld - N; n += 2) du.p[m * du.ld + n] = f2bf(0.f);
   }
 };
 
