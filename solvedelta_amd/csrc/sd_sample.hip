@@ -283,9 +283,12 @@ template <class E, int T> struct SampleRow {
   float R, c;   // masses are 2^((l - R) c)
   static constexpr int N = LogitVec<E>::N, G = 16 / N;
   __device__ __forceinline__ float expo(float l) const { return (l - R) * c; }
-  // 64 bins an octave of the mass, from 2^12 down to 2^-52; the last takes what is behind
+  // 64 bins an octave of the mass, from 2^12 down to 2^-52; the last takes what is behind.  A
+  // token is looked for in the bin where it was counted: the multiply-add is written out, since
+  // the compiler would fuse kOver - expo in one place and not in another, which at a bin's edge
+  // are different bins (20 of 10^6 FP32 logits).
   __device__ __forceinline__ int bin(float l) const {
-    const int b = (int)fminf((kOver - expo(l)) * 64.f, (float)(SMP_BINS - 1));
+    const int b = (int)fminf(__builtin_fmaf(expo(l), -64.f, kOver * 64.f), (float)(SMP_BINS - 1));
     return b < 0 ? 0 : b;
   }
   // x 2^30, rounded: whole part and fraction of x 2^-2 as the two halves (x up to 2^13)
