@@ -137,7 +137,8 @@ int sd_linear_int8(int64_t N, int K, int O, const void *x, int64_t x_st, const i
  * sum exp(z) (all if top_p >= 1), of these those with z >= log(min_p) (all if min_p <= 0).
  * token[b]: the kept token with the largest z - log(-log noise), the lowest index of equals;
  * at a temperature that is not positive, rank 0; -1 if every logit is -infinity or NaN.
- * V <= 2^22. */
+ * Masses are FP32 exponentials, each within 2^-17 of itself down to 2^-52 of the largest, and
+ * their sums are right to 2^-28 of the largest.  V <= 2^22. */
 typedef struct {
   double value;
   const void *rows;

@@ -18,8 +18,9 @@
 // For top_k <= 256 one atomic a thread is enough: the k-th largest of the threads' own maxima
 // bounds the k-th largest logit from below, and what reaches it is listed and ranked.
 //
-// Masses are 64-bit fixed point, summed in any order to the same bits: every call gives the
-// same token.  As -log u >= 1 - u, a token whose (1 - u) exp(-z) is more than 8 times the
+// Masses are whole numbers, summed in any order to the same bits: every call gives the
+// same token.  Each octave of masses has a unit of its own, in which an FP32 exponential is
+// exact: a light token weighs what it does, however many there are.  As -log u >= 1 - u, a token whose (1 - u) exp(-z) is more than 8 times the
 // workgroup's best so far needs no logarithm, and as -log u <= 2 (1 - u) for u >= 1/4 that
 // best is bounded before the first one is taken.
 #include <hip/hip_runtime.h>
@@ -36,8 +37,7 @@ constexpr int SMP_FIRST = 512;  // threads whose first tokens give R, however ma
 constexpr int kMaxVocab = 1 << 22;
 constexpr float kInf = __builtin_inff();
 // Masses are 2^((l - R) c): R is the maximum of the row's first tokens, and the row's own may
-// be up to 2^12 masses above it (else the pass is run again with R the maximum).  In units of
-// 2^-30, 2^22 of them stay below 2^64.
+// be up to 2^12 masses above it (else the pass is run again with R the maximum).
 constexpr float kOver = 12.f;
 
 // ranks: a larger key is drawn from first
@@ -135,7 +135,7 @@ template <int T> struct SampleLds {
   u64 hist[SMP_BINS];
   u64 key[T], mass[T];
   u64 red[T / 64];
-  u64 before, cut;
+  u64 rest, cut;
   int bin, n;
   unsigned bound;  // the race's best time so far
 };
@@ -194,14 +194,35 @@ template <int T> __device__ __forceinline__ void clear_hist() {
   if (threadIdx.x == 0) s.n = 0;
 }
 
+// Masses of the d-th octave from the peak's are whole numbers up to 2^31 in units of its own;
+// up to 2^22 of them, in units that all octaves share (2^-41 of the largest mass there can be in the
+// peak's octave), sum to less than 2^64.  What is cut off is less than one unit a bin: 2^-28 of the
+// peak's mass in all.
+constexpr int SMP_SHARED = 10;
+__device__ __forceinline__ u64 to_shared(u64 sum, int d) {
+  return d <= SMP_SHARED ? sum << (SMP_SHARED - d) : sum >> (d - SMP_SHARED);
+}
+// the least sum in the octave's own units that is x or more in shared ones
+__device__ __forceinline__ u64 to_own(u64 x, int d) {
+  const int k = SMP_SHARED - d;
+  return k >= 0 ? (x + ((u64)1 << k) - 1) >> k : x << -k;
+}
+
 // The first bin whose inclusive sum, counted from bin 0, reaches target(sum of all): s.bin,
-// and the sum before it in s.before.  Returns the target; 0 where the sum of all is less.
-template <int T, class F> __device__ __forceinline__ u64 find_bin(F target_of) {
+// and what is left of the target there in s.rest.  Returns the target; 0 where the sum of all is
+// less.  first: the peak's octave where the bins hold masses, -1 where they hold numbers.
+template <int T, class F> __device__ __forceinline__ u64 find_bin(int first, F target_of) {
   SampleLds<T>& s = smp_lds<T>();
   constexpr int PER = SMP_BINS / T;
+  static_assert(64 % PER == 0, "a thread's bins are of one octave");
+  const int octave = (int)threadIdx.x * PER >> 6, d = octave > first ? octave - first : 0;
   u64 h[PER], own = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) { h[i] = s.hist[threadIdx.x * PER + i]; own += h[i]; }
+  for (int i = 0; i < PER; ++i) {
+    h[i] = s.hist[threadIdx.x * PER + i];
+    if (first >= 0) h[i] = to_shared(h[i], d);
+    own += h[i];
+  }
   const u64 inc = wave_scan<OpSum>(own);
   __syncthreads();  // s.red may still be read by a wave behind
   if (lane_id() == 63) s.red[wave_id()] = inc;
@@ -220,7 +241,7 @@ template <int T, class F> __device__ __forceinline__ u64 find_bin(F target_of) {
     for (int e = 0; e < PER - 1; ++e)
       if (i == e && acc + h[e] < target) { acc += h[e]; i = e + 1; }
     s.bin = threadIdx.x * PER + i;
-    s.before = acc;
+    s.rest = first >= 0 ? to_own(target - acc, d) : target - acc;
   }
   __syncthreads();
   return all < target ? 0 : target;
@@ -291,15 +312,14 @@ template <class E, int T> struct SampleRow {
     const int b = (int)fminf(__builtin_fmaf(expo(l), -64.f, kOver * 64.f), (float)(SMP_BINS - 1));
     return b < 0 ? 0 : b;
   }
-  // x 2^30, rounded: whole part and fraction of x 2^-2 as the two halves (x up to 2^13)
-  static __device__ __forceinline__ u64 fixed(float x) {
-    const float y = x * 0.25f, f = __builtin_amdgcn_fractf(y);
-    const u64 lo = (u64)(unsigned)y << 32;
-    return lo + (unsigned)fminf(__builtin_fmaf(f, 4294967296.f, 0.5f), 4294967040.f);
+  // A mass x in bin b, in units of its octave's, from 2^30 to 2^31 of them (the last octave has the
+  // lighter ones too): FP32's 24 bits are all whole ones.
+  static __device__ __forceinline__ unsigned units(float x, int b) {
+    return (unsigned)__builtin_amdgcn_ldexpf(x, 31 - (int)kOver + (b >> 6));
   }
-  __device__ __forceinline__ u64 mass(float l) const { return fixed(fmaxf(__builtin_amdgcn_exp2f(expo(l)), 0.f)); }
-  __device__ __forceinline__ u64 term(int hist, float l) const {
-    return hist == HIST_MASS ? mass(l) : l > -kInf ? 1ull : 0ull;
+  __device__ __forceinline__ float mass(float l) const { return fmaxf(__builtin_amdgcn_exp2f(expo(l)), 0.f); }
+  __device__ __forceinline__ unsigned term(int hist, float l, int b) const {
+    return hist == HIST_MASS ? units(mass(l), b) : l > -kInf ? 1u : 0u;
   }
   // the race's time as a key, smaller is better, with the index behind it
   __device__ __forceinline__ u64 time(int v, float l, float u) const {
@@ -324,8 +344,9 @@ template <class E, int T> struct SampleRow {
     };
     auto count = [&](int v, float l, float x) {
       if (CUT && !in.keeps(l, v)) return;
-      const u64 m = hist == HIST_MASS ? fixed(x) : l > -kInf ? 1ull : 0ull;
-      if (m) atomicAdd(&s.hist[bin(l)], m);
+      const int at = bin(l);
+      const unsigned m = hist == HIST_MASS ? units(x, at) : l > -kInf ? 1u : 0u;
+      if (m) atomicAdd(&s.hist[at], (u64)m);
     };
     row.template groups<G>(
         [&](int v0, const u4v(&y)[G], int n) {
@@ -354,7 +375,7 @@ template <class E, int T> struct SampleRow {
 #pragma unroll
               for (int e = 0; e < N; ++e) {
                 const float l = row.value(LogitVec<E>::at(y[i], e));
-                count(v0 + i * T * N + e, l, hist == HIST_MASS ? fmaxf(__builtin_amdgcn_exp2f(expo(l)), 0.f) : 0.f);
+                count(v0 + i * T * N + e, l, hist == HIST_MASS ? mass(l) : 0.f);
               }
             }
             // a better bound on the race's best time, before any logarithm (at a row's end the
@@ -382,7 +403,7 @@ template <class E, int T> struct SampleRow {
         },
         [&](int v, float l) {
           mx = fmaxf(mx, l);
-          if (hist) count(v, l, fmaxf(__builtin_amdgcn_exp2f(expo(l)), 0.f));
+          if (hist) count(v, l, mass(l));
           one(v, l, noise[v]);
         });
     *top = mx;
@@ -440,10 +461,10 @@ template <class E, int T> struct SampleRow {
   }
 };
 
-// The smallest of the keys in [lo, hi] whose inclusive sum of `term` over larger keys, on top
-// of `before`, reaches the target: 8 bits at a time from the first in which lo and hi differ.
+// The smallest of the keys in [lo, hi], all of one bin, whose inclusive sum of `term` over larger
+// keys reaches `rest`: 8 bits at a time from the first in which lo and hi differ.
 template <class E, int T>
-__device__ __forceinline__ u64 radix_cut(const SampleRow<E, T> r, int hist, u64 lo, u64 hi, u64 before, u64 target) {
+__device__ __forceinline__ u64 radix_cut(const SampleRow<E, T> r, int hist, int bin, u64 lo, u64 hi, u64 rest) {
   SampleLds<T>& s = smp_lds<T>();
   int top = lo == hi ? 0 : 64 - __clzll((long long)(lo ^ hi));  // bits that may differ
   u64 prefix = top >= 64 ? 0 : hi >> top;
@@ -454,31 +475,30 @@ __device__ __forceinline__ u64 radix_cut(const SampleRow<E, T> r, int hist, u64 
     r.row.each([&](int v, float l) {
       const u64 key = rank_key(l, v);
       if (key < lo || key > hi || (top < 64 && key >> top != prefix)) return;
-      const u64 m = r.term(hist, l);
-      if (m) atomicAdd(&s.hist[(key >> shift) & ((1 << nbits) - 1)], m);
+      const unsigned m = r.term(hist, l, bin);
+      if (m) atomicAdd(&s.hist[(key >> shift) & ((1 << nbits) - 1)], (u64)m);
     });
     __syncthreads();
     if (threadIdx.x == 0) {
       int d = (1 << nbits) - 1;
-      u64 acc = before;
-      while (d > 0 && acc + s.hist[d] < target) acc += s.hist[d--];
+      u64 acc = 0;
+      while (d > 0 && acc + s.hist[d] < rest) acc += s.hist[d--];
       s.bin = d;
-      s.before = acc;
+      s.rest = rest - acc;
     }
     __syncthreads();
     prefix = (prefix << nbits) | (u64)s.bin;
-    before = s.before;
+    rest = s.rest;
     top = shift;
     __syncthreads();
   }
   return prefix;
 }
 
-// The key inside `bin` of the tokens that `in` keeps at which the sum of their terms, on top
-// of `before`, reaches the target.
+// The key inside `bin` of the tokens that `in` keeps at which the sum of their terms reaches
+// `rest`.
 template <class E, int T>
-__device__ __forceinline__ SampleCut exact_cut(const SampleRow<E, T> r, int hist, const SampleCut in, int bin, u64 before,
-                                            u64 target) {
+__device__ __forceinline__ SampleCut exact_cut(const SampleRow<E, T> r, int hist, const SampleCut in, int bin, u64 rest) {
   SampleLds<T>& s = smp_lds<T>();
   __syncthreads();
   if (threadIdx.x == 0) s.n = 0;
@@ -486,7 +506,7 @@ __device__ __forceinline__ SampleCut exact_cut(const SampleRow<E, T> r, int hist
   u64 lo = ~0ull, hi = 0;
   r.row.each([&](int v, float l) {
     if (r.bin(l) != bin || !in.keeps(l, v)) return;
-    const u64 m = r.term(hist, l);
+    const unsigned m = r.term(hist, l, bin);
     if (!m) return;
     const u64 key = rank_key(l, v);
     lo = key < lo ? key : lo;
@@ -500,10 +520,10 @@ __device__ __forceinline__ SampleCut exact_cut(const SampleRow<E, T> r, int hist
   if (n <= T) {
     if ((int)threadIdx.x < n) {
       const u64 own = s.key[threadIdx.x];
-      u64 acc = before;
+      u64 acc = 0;
 #pragma unroll 4
       for (int j = 0; j < n; ++j) acc += s.key[j] > own ? s.mass[j] : 0;
-      if (acc < target && acc + s.mass[threadIdx.x] >= target) s.cut = own;
+      if (acc < rest && acc + s.mass[threadIdx.x] >= rest) s.cut = own;
     }
     __syncthreads();
     key = s.cut;
@@ -511,7 +531,7 @@ __device__ __forceinline__ SampleCut exact_cut(const SampleRow<E, T> r, int hist
   } else {
     lo = ~block_max<T>(~lo);
     hi = block_max<T>(hi);
-    key = radix_cut(r, hist, lo, hi, before, target);
+    key = radix_cut(r, hist, bin, lo, hi, rest);
   }
   return {key_logit(key), key_index(key)};
 }
@@ -535,12 +555,13 @@ __device__ __forceinline__ u64 draw_listed(const SampleRow<E, T> r, float own, i
   if (own > -kInf) atomicAdd(&s.hist[octave_bin(r.R - own)], 1ull);
   __syncthreads();
   // bin b holds edge(b) <= d < edge(b + 1)
-  const bool some = find_bin<T>([&](u64) { return (u64)k; }) != 0;
+  const bool some = find_bin<T>(-1, [&](u64) { return (u64)k; }) != 0;
   const float to = some && s.bin < SMP_BINS - 1 ? __uint_as_float((unsigned)(s.bin + 1 + kBinOff) << 16) : kInf;
   auto list = [&](int v, float l) {
     if (!(r.R - l < to)) return;
     const int at = atomicAdd(&s.n, 1);
-    if (at < T) { s.key[at] = rank_key(l, v); s.mass[at] = r.mass(l); }
+    // masses up to 1, of which 2^-52 is left
+    if (at < T) { s.key[at] = rank_key(l, v); s.mass[at] = (u64)(r.mass(l) * 0x1p52f); }
   };
   typedef LogitVec<E> L;
   r.row.template groups<4>(
@@ -676,16 +697,17 @@ __global__ __launch_bounds__(T, 4) void k_sample(SampleArgs a) {
         break;
       }
     }
-    target = hist ? find_bin<T>([&](u64 total) { return hist == HIST_COUNT ? (u64)k : target_of(p, total); }) : 0;
-    if (stage == 0 && by_p && target) in = exact_cut(r, HIST_COUNT, all, s.bin, s.before, target);
+    const int first = hist == HIST_MASS ? r.bin(peak) >> 6 : -1;
+    target = hist ? find_bin<T>(first, [&](u64 total) { return hist == HIST_COUNT ? (u64)k : target_of(p, total); }) : 0;
+    if (stage == 0 && by_p && target) in = exact_cut(r, HIST_COUNT, all, s.bin, s.rest);
   }
   SampleKept kept{SMP_BINS, in, peak, dmax};
-  const u64 before = s.before;
+  const u64 rest = s.rest;
   if (target) kept.bin = s.bin;
   float over = __uint_as_float(s.bound) * kPass, l;
   u64 best = r.fastest(kept, two, over, &l);
   if (target && r.bin(l) == kept.bin) {
-    kept.cut = exact_cut(r, by_p ? HIST_MASS : HIST_COUNT, in, kept.bin, before, target);
+    kept.cut = exact_cut(r, by_p ? HIST_MASS : HIST_COUNT, in, kept.bin, rest);
     best = r.fastest(kept, two, over, &l);
   }
   if (threadIdx.x == 0) a.token[b] = (int)(unsigned)best;

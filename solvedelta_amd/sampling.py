@@ -61,6 +61,7 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, temperature: Settin
     softmax over the kept tokens.  temperature 0 takes the first token;
     top_k <= 0, top_p >= 1 and min_p <= 0 switch a filter off.  Logits of -infinity
     or NaN are never drawn; a row that holds nothing else gives -1.
+    Masses are FP32 exponentials, summed to 2^-28 of the largest.
 
     Entries of setting tensors are not checked (that would wait for the GPU): a
     temperature that is not positive reads as 0.
