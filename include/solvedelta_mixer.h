@@ -122,7 +122,7 @@ int sd_quantize_int8(int64_t N, int K, int is_fp32, const void *x, int64_t x_st,
                      int64_t q_st, float *scale, void *stream);
 /* y[n,o] = s_n w_scale[o] sum_k q[n,k] w[o,k] + bias[o], (q, s) the rows of x quantised as
  * above.  x: bf16 [N][K], row stride x_st; w: int8 [O][K], row stride w_st; bias: bf16 [O],
- * nullable; y: bf16 [N][O] contiguous.  K <= 133144: sums stay within 32 bits. */
+ * nullable; y: bf16 [N][O] contiguous.  K <= 132104: sums stay within 32 bits, of weights of -128 too. */
 size_t sd_linear_int8_workspace_bytes(int64_t N, int K, int O, const void *w, int64_t w_st);
 int sd_linear_int8(int64_t N, int K, int O, const void *x, int64_t x_st, const int8_t *w,
                    int64_t w_st, const float *w_scale, const void *bias, void *y,

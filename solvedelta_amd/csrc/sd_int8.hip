@@ -1,7 +1,7 @@
 // 8-bit integer linear layer: tokens quantised row by row,
 //   s_n = max_k |x_nk| / 127, q_nk = rint(x_nk / s_n) (a zero row: s_n = 0, q = 0),
 //   y_no = s_n w_o sum_k q_nk W_ok (+ bias_o),
-// sums in 32-bit integers (exact up to K = 2^31 / 127^2), scales FP32.  A row that holds an
+// sums in 32-bit integers (exact up to K = 2^31 / (127 * 128)), scales FP32.  A row that holds an
 // infinity or a NaN has the scale NaN and comes out NaN.
 #include <hip/hip_runtime.h>
 
@@ -267,7 +267,7 @@ using Tile = GemmTile<int8_t, 2, TILE == 0 ? 4 : TILE == 3 ? 1 : 2, TILE == 0 ? 
 
 GemmPlan plan_int8(int64_t N, int K, int O) { return plan_gemm(N, O, (K + 127) / 128); }
 
-constexpr int kMaxK = 133144;       // 2^31 / 127^2
+constexpr int kMaxK = 132104;       // 2^31 / (127 * 128): a weight may be -128
 constexpr int64_t kMaxRow = 1 << 22;  // bytes between a weight's rows: a tile's offsets stay in 31 bits
 bool int8_shape_ok(int64_t N, int K, int O) {
   return N > 0 && K > 0 && O > 0 && K <= kMaxK && N < (int64_t(1) << 30) &&
