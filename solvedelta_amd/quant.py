@@ -65,7 +65,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     O, K = weight.shape
     if weight_scale.shape != (O,) or (bias is not None and bias.shape != (O,)):
         raise ValueError("weight_scale and bias must have shape [O]")
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
         raise RuntimeError("int8_linear has no backward: call it under torch.no_grad()")
     dev = x.device
     y = torch.empty((*x.shape[:-1], O), dtype=torch.bfloat16, device=dev)
