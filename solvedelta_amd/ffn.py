@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .operator import _call, _ptr
+from .operator import _call, _has_tangent, _ptr
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -87,7 +87,7 @@ def gated_ffn(x: torch.Tensor, gate_up_weight: torch.Tensor,
 
     x [..., D]; gate_up_weight [2 I, D], the gate's rows first; down_weight
     [O, I].  Returns [..., O].  Rows may be strided; gradients flow to all
-    three arguments (once: no double backward).  What the backward reads is
+    three arguments (once: no double backward, and no forward mode).  What the backward reads is
     kept in 16 bits, 6 I bytes a token and a little more.
     """
     for t in (x, gate_up_weight, down_weight):
@@ -103,6 +103,8 @@ def gated_ffn(x: torch.Tensor, gate_up_weight: torch.Tensor,
     if gate_up_weight.shape != (2 * I, x.shape[-1]) or not I or not O or not x.shape[-1]:
         raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, gate_up_weight "
                          f"{tuple(gate_up_weight.shape)}, down_weight {tuple(down_weight.shape)}")
+    if _has_tangent(x, gate_up_weight, down_weight):
+        raise RuntimeError("gated_ffn has no forward-mode derivative")
     grad = torch.is_grad_enabled() and (x.requires_grad or gate_up_weight.requires_grad
                                         or down_weight.requires_grad)
     if not x.numel():   # no tokens: an empty result with zero gradients

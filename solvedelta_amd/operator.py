@@ -12,6 +12,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .state import SolveDeltaState
@@ -69,6 +70,12 @@ def _call(fn, device: torch.device, *args) -> int:
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
+
+
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether forward-mode differentiation runs and one of these carries a tangent."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _SolveDeltaFn(torch.autograd.Function):

@@ -13,7 +13,7 @@ from torch import nn
 
 from . import _lib
 from .ffn import _row_stride, _rows
-from .operator import _call, _ptr
+from .operator import _call, _has_tangent, _ptr
 
 
 def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -68,6 +68,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad
                                     or (bias is not None and bias.requires_grad)):
         raise RuntimeError("int8_linear has no backward: call it under torch.no_grad()")
+    if _has_tangent(x, weight_scale, bias):
+        raise RuntimeError("int8_linear has no forward-mode derivative")
     dev = x.device
     y = torch.empty((*x.shape[:-1], O), dtype=torch.bfloat16, device=dev)
     if not x.numel():

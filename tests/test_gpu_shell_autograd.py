@@ -1,6 +1,7 @@
 """Derivatives that the causal LM's operators do not have are refused, not dropped."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -19,3 +20,22 @@ def test_int8_linear_has_no_gradient_for_its_scales():
             int8_linear(args[0], w, args[1], args[2])
         with torch.no_grad():
             assert not int8_linear(args[0], w, args[1], args[2]).requires_grad
+
+
+@pytest.mark.parametrize("N", [0, 3])
+def test_forward_mode_is_refused(N):
+    from solvedelta_amd import gated_ffn, int8_linear
+    ffn = (_z(N, 8), _z(8, 8), _z(8, 4))
+    int8 = (_z(N, 8), _z(4, dtype=torch.float32), _z(4))
+    w = _z(4, 8, dtype=torch.int8)
+    with forward_ad.dual_level():
+        gated_ffn(*ffn)             # nothing to differentiate
+        int8_linear(int8[0], w, *int8[1:])
+        for i in range(3):
+            for grad in (False, True):
+                with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError)):
+                    gated_ffn(*(forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t
+                                for j, t in enumerate(ffn)))
+            a = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(int8)]
+            with pytest.raises(RuntimeError):
+                int8_linear(a[0], w, a[1], a[2])
