@@ -40,11 +40,19 @@ class SolveDeltaLMConfig(SolveDeltaMixerConfig):
     fused_ffn: bool = False
 
 
+def _only_its_weight(proj: nn.Module) -> bool:
+    """Whether calling ``proj`` is the product with its weight and nothing else."""
+    return (type(proj) is nn.Linear and proj.bias is None and "forward" not in vars(proj)
+            and not (proj._forward_hooks or proj._forward_pre_hooks or proj._backward_hooks
+                     or proj._backward_pre_hooks))
+
+
 class SolveDeltaMLP(nn.Module):
     """SwiGLU MLP with one gate/up projection (modeling_solvedelta.py:31-100).
 
     ``fused``: the whole block runs as ``gated_ffn``, in bf16 (parameters in bf16, or
-    under bf16 autocast); projections that were put in 8 bits run on their own."""
+    under bf16 autocast); projections that were put in 8 bits, have a bias, hooks or a
+    forward of their own run on their own."""
 
     def __init__(self, hidden_size: int, hidden_ratio: Optional[int] = None,
                  intermediate_size: Optional[int] = None, fused: bool = False) -> None:
@@ -61,7 +69,8 @@ class SolveDeltaMLP(nn.Module):
         self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False)
 
     def forward(self, x):
-        if self.fused and type(self.gate_up_proj) is type(self.down_proj) is nn.Linear:
+        if (self.fused and _only_its_weight(self.gate_up_proj) and _only_its_weight(self.down_proj)
+                and not nn.modules.module._has_any_global_hook()):
             args = x, self.gate_up_proj.weight, self.down_proj.weight
             if x.is_cuda and torch.is_autocast_enabled("cuda"):
                 dtype = torch.get_autocast_dtype("cuda")
