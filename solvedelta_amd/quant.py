@@ -88,7 +88,10 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
 
 class Int8Linear(nn.Module):
-    """A Linear whose weight is held in 8 bits, for inference."""
+    """A Linear whose weight is held in 8 bits, for inference.
+
+    Its buffers follow the module from device to device but keep their types: a cast of
+    the model would round the scales, and the product takes no others."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = False, *,
                  device=None) -> None:
@@ -110,6 +113,12 @@ class Int8Linear(nn.Module):
         if linear.bias is not None:
             q.bias = linear.bias.detach().to(torch.bfloat16)
         return q
+
+    def _apply(self, fn, recurse=True):
+        # casts change floating tensors alone: they see the bits
+        bits = {torch.float32: torch.int32, torch.bfloat16: torch.int16}
+        return super()._apply(lambda t: fn(t.view(bits[t.dtype])).view(t.dtype) if t.dtype in bits
+                              else fn(t), recurse)
 
     def forward(self, x):
         return int8_linear(x.to(torch.bfloat16), self.weight, self.weight_scale, self.bias)
