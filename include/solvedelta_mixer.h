@@ -128,6 +128,11 @@ int sd_linear_int8(int64_t N, int K, int O, const void *x, int64_t x_st, const i
                    int64_t w_st, const float *w_scale, const void *bias, void *y,
                    void *workspace, size_t workspace_bytes, void *stream);
 
+/* How a product of M x N outputs and rows of k_bytes is cut, for tests and profiles.  plan[0]: the
+ * tile, 0 is 256x256, 1 and 2 are 128x128, 3 is 64x64; plan[1]: how many tiles are done whole;
+ * plan[2]: how many workgroups share the others, which a second kernel joins. */
+int sd_product_plan(int64_t M, int64_t N, int64_t k_bytes, int plan[3]);
+
 /* One token per row of logits [B][V] (bf16, or FP32 if is_fp32; row stride logits_st), from
  * uniform numbers noise [B][V] (FP32, row stride noise_st; read between 2^-25 and 1 - 2^-24).
  * settings: temperature, top_k, top_p, min_p, in this order; each is `value` for all rows, or

@@ -115,6 +115,7 @@ EXPORTS = {
     "sd_linear_int8": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                       ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]
                        + [ctypes.c_void_p] * 4 + [ctypes.c_size_t, ctypes.c_void_p]),
+    "sd_product_plan": (ctypes.c_int, [ctypes.c_int64] * 3 + [ctypes.c_int * 3]),
     "sd_sample_tokens": (ctypes.c_int, [ctypes.c_int] * 3 + [ctypes.c_void_p, ctypes.c_int64] * 2
                          + [ctypes.POINTER(SdSampleSetting)] + [ctypes.c_void_p] * 2),
 }

@@ -275,6 +275,14 @@ using namespace sd;
 
 extern "C" {
 
+int sd_product_plan(int64_t M, int64_t N, int64_t k_bytes, int plan[3]) {
+  if (M <= 0 || N <= 0 || k_bytes <= 0 || M > INT32_MAX || N > INT32_MAX || k_bytes > INT32_MAX) return SD_ERR_SHAPE;
+  if (!plan) return SD_ERR_ARG;
+  const GemmPlan p = plan_gemm(M, N, (k_bytes + 127) / 128);
+  plan[0] = p.tile; plan[1] = p.whole; plan[2] = p.workers;
+  return SD_OK;
+}
+
 size_t sd_ffn_saved_bytes(const sd_ffn* f) {
   if (!ffn_shape_ok(f)) return 0;
   return saved_blocks_bytes(*f) + a_bytes(*f);
