@@ -136,10 +136,11 @@ struct SkinnyOut {
 namespace {
 
 typedef __bf16 bf;
-// Straight from memory to MFMA each workgroup of 8 columns reads all tokens: up to 64 tokens
-// and 200 MB of such reads in all that is the faster way (22.4 us for one token of D=2048
-// I=5632, 28.6 for 16; the 64x64 tile 28.5 and 29.4), beyond it the tile is (32 tokens: 29.5
-// against 37.8 us; 64 tokens of D=1024 I=2816, 92 MB: 22.5 against 20.9).
+// Straight from memory to MFMA each workgroup of 8 columns reads all tokens, N I (D + O) / 4 bytes
+// in all.  Up to 64 tokens and 100 MB of such reads that is the faster way, beyond it the 64x64 tile
+// is.  In a graph, with the weights in memory and (in brackets) in the caches, straight and tile:
+// one token of D=2048 I=5632 23.4 and 31.3 us (19.1, 28.2), 16 (92 MB) 29.3 and 31.6 (26.3, 28.3), 24
+// (138 MB) 35.0 and 31.9 (32.2, 28.5); 64 of D=1024 I=2816 (92 MB) 22.2 and 23.9 (20.3, 22.1).
 bool few(const sd_ffn& f) { return f.N <= 64 && f.N * f.I * ((int64_t)f.D + f.O) <= 400000000; }
 
 template <int NT>

@@ -274,14 +274,21 @@ bool int8_shape_ok(int64_t N, int K, int O) {
          (N / 128 + 1) * ((int64_t)O / 128 + 1) < (1 << 23);
 }
 
-// Columns a workgroup of few tokens: 64, 16 or 8, as many as leave one for every CU twice.
+// Columns a workgroup of few tokens: 64, 16 or 8, the most that leave a workgroup for each of 256
+// CUs.  One token, with the weights in memory: K=1024 O=32000 10.3 us with 64, 18.8 with 16; O=5632 5.6
+// with 16, 6.4 with 64, 8.2 with 8; K=2048 O=2048 5.7 with 8, 8.9 with 64; O=11264 12.0 with 16
+// (10.3 with 64, which would leave 80 CUs idle: the cut is a little late there).
 int few_cols(int O) { return O >= 64 * 512 / 2 ? 64 : O >= 16 * 256 ? 16 : 8; }
 
 // Tokens that every workgroup quantises for itself, where that costs less than the launch of
-// k_quant: one token of K=2048 O=11264 takes 11.5 us so and 13.5 else, four 21.9 and 13.4.
+// k_quant: one token of K=2048 O=11264 takes 11.5 us so and 13.5 else, four 21.9 and 13.4.  (In a
+// graph, where launches cost less, two take 15.3 so, and four take 11.0 by the launch.)
 bool fused(int64_t N, int K) { return N <= 2 && N * (up(K, 128) + 16) <= 8192 + 32; }
-// Quantised tokens straight from memory to MFMA: up to 32 (K=1024 O=32000: 15.2 us against
-// the 64x64 tile's 16.4), up to 64 where O is narrow (64 of K=5632 O=2048: 24.2 against 27.2).
+// Quantised tokens straight from memory to MFMA: up to 32, up to 64 where O is narrow.  In a graph,
+// with the weights in memory, so and by the 64x64 tile: 16 of K=1024 O=32000 12.3 and 15.3 us, 32 15.9
+// and 15.6; 32 of K=1024 O=5632 8.6 and 11.5; 64 of K=2048 O=2048 11.8 and 15.1.  The tile is ahead
+// where the tokens' own reads weigh more: 32 of K=2048 O=11264 18.3 and 15.4, 64 of K=5632 O=2048 27.2
+// and 24.7.
 bool few(int64_t N, int O) { return N <= 32 || (N <= 64 && O < 4096); }
 
 template <int R, int U, bool HALF>

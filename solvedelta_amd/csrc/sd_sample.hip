@@ -714,9 +714,9 @@ __global__ __launch_bounds__(T, 4) void k_sample(SampleArgs a) {
 }
 
 // Rows of 1024 threads have a CU to themselves; of 512, two share one, and one's loads and
-// arithmetic run in the other's waits.  512 x 50001 FP32: 40.3 and 34.3 us without a filter, 39.3 and
-// 34.3 at top_k 50, 54.7 and 45.8 at top_p 0.9; 2048 x 32000 bf16: 107 and 77, 85 and 57, 156 and 108;
-// 257 x 50001: 31 and 25, 30 and 23, 42 and 35 (the other way only at min_p, 30 and 34).  The token
+// arithmetic run in the other's waits.  512 x 50001 FP32, in a graph: 40.9 and 35.1 us without a
+// filter, 39.0 and 34.5 at top_k 50, 54.8 and 50.4 at top_p 0.9; 2048 x 32000 bf16: 108 and 81, 85 and
+// 57, 149 and 107; 257 x 50001: 32 and 26, 31 and 24, 43 and 36 (32 and 32 at min_p).  The token
 // is the same.
 template <class E> void launch_sample(int B, const SampleArgs& a, hipStream_t st) {
   if (B > 256) SD_LAUNCH("k_sample", (k_sample<E, 512>), dim3(B), dim3(512), 0, st, a);

@@ -21,7 +21,7 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
     scale = max |x| / 127 over the row, q = rint(x / scale); a zero row has scale
     0 and q 0, a row that holds an infinity or a NaN the scale NaN.  x is bf16 or
-    FP32 on a ROCm device."""
+    FP32 on a ROCm device; the results are detached from it."""
     if not x.is_cuda:
         raise TypeError("quantize_int8 runs on a ROCm device only")
     if x.dtype not in (torch.bfloat16, torch.float32):
